@@ -151,7 +151,8 @@ def check_writes(g: Graph) -> None:
 
     Every write has to reach an output (a program computes what is returned), its operand has to
     be an argument of the program or an earlier write's result, and nothing else may read the
-    operand: a reader of the value before the write has no order with it."""
+    operand, as it is or reshaped, nor may the write's other operands be it: a reader of the value
+    before the write has no order with it."""
     writes = [n for n in g.nodes if n.op in IN_PLACE]
     if not writes:
         return
@@ -166,7 +167,8 @@ def check_writes(g: Graph) -> None:
     for w in writes:
         if id(w) not in live:
             raise ValueError(f"{w.op}: the result must be returned, or read by what is returned")
-        before = _unshaped(w.inputs[IN_PLACE[w.op]])
+        place = IN_PLACE[w.op]
+        before = _unshaped(w.inputs[place])
         if before.op != "input" and before.op not in IN_PLACE:
             raise ValueError(f"{w.op} writes into its first operand: it must be an argument of the function or the "
                              f"result of another {w.op}, not of {before.op}")
@@ -180,7 +182,7 @@ def check_writes(g: Graph) -> None:
                     continue
                 if u.op == "reshape":
                     values.append(u)
-                elif u is not w or sum(i is v for i in u.inputs) > 1:
+                elif u is not w or any(i is v for j, i in enumerate(w.inputs) if j != place):
                     readers.append(u.op)
         if readers:
             raise ValueError(f"{w.op}: the cache is also read by {', '.join(sorted(set(readers)))} without the write: "

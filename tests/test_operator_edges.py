@@ -1,0 +1,61 @@
+"""Operators without a GPU: calls at the edge of what they accept."""
+import pytest
+
+import tensorjit as tj
+from tensorjit.compiler import lower
+from tensorjit.ir import DType, TensorType
+
+
+def T(*shape, dt="bf16"):
+    return TensorType(shape, DType(dt))
+
+
+def trace(fn, *types):
+    return tj.trace(fn, list(types))
+
+
+CACHE, NEW, PAGES, SEQ = T(10, 4, 3, 24), T(2, 5, 3, 24), T(2, 6, dt="i32"), T(2, dt="i32")
+
+
+# ---------------------------------------------------------------------------
+# writes in place
+# ---------------------------------------------------------------------------
+
+
+def test_a_write_does_not_read_its_own_cache():
+    """As it is, reshaped on either side, through two reshapes, and of a write's result."""
+    def same(c, x, p, s):
+        return tj.paged_write(c, c, p, s)
+
+    def rows(c, x, p, s):
+        return tj.paged_write(c, tj.reshape(c, 2, 20, 3, 24), p, s)
+
+    def cache(c, x, p, s):
+        return tj.paged_write(tj.reshape(c, 10, 4, 3, 24), c, p, s)
+
+    def both(c, x, p, s):
+        return tj.paged_write(tj.reshape(c, 10, 4, 3, 24), tj.reshape(tj.reshape(c, 40, 72), 2, 20, 3, 24), p, s)
+
+    def chained(c, x, p, s):
+        first = tj.paged_write(c, x, p, s)
+        return tj.paged_write(first, tj.reshape(first, 2, 20, 3, 24), p, s)
+
+    def chained_cache(c, x, p, s):
+        first = tj.paged_write(c, x, p, s)
+        return tj.paged_write(tj.reshape(first, 10, 4, 3, 24), tj.reshape(first, 2, 20, 3, 24), p, s)
+
+    as_rows = T(2, 20, 3, 24)
+    for fn, kind in ((same, as_rows), (rows, CACHE), (cache, as_rows), (both, CACHE), (both, T(10, 4, 72)), (chained, CACHE),
+                     (chained_cache, CACHE)):
+        with pytest.raises(ValueError, match="read the result"):
+            lower(trace(fn, kind, NEW, PAGES, SEQ))
+
+
+def test_a_reshaped_cache_is_written_once():
+    """Reshapes of the destination alone stay allowed."""
+    def f(c, x, p, s):
+        first = tj.paged_write(tj.reshape(c, 10, 4, 3, 24), x, p, s)
+        return tj.paged_write(tj.reshape(tj.reshape(first, 40, 72), 10, 4, 3, 24), x + 1.0, p, s)
+
+    program = lower(trace(f, T(10, 4, 72), NEW, PAGES, SEQ))
+    assert program.storage(program.graph.outputs[0]) is program.graph.inputs[0]
