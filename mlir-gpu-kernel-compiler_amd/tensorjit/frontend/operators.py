@@ -108,7 +108,7 @@ def paged_attention(q: Tensor, k: Tensor, v: Tensor, pages: Tensor, starts: Tens
     dim]``; consecutive groups of ``query heads / heads`` query heads share a head of the caches.
     Query ``i < counts[b]`` (default: all ``S``) of sequence ``b`` stands at position ``t =
     starts[b] + i`` and sees the keys at positions ``0 .. t``, with ``window`` the last ``window`` of
-    them (itself included).  ``scale`` (default ``dim ** -0.5``) must be positive.
+    them (itself included).  ``scale`` (default ``dim ** -0.5``) must be from 1e-30 to 1e30.
 
     Keys past the page table, or in a page that is not one of the cache's, are left out.  A query
     that sees no key gives zeros, and so do one whose scores are all ``-inf`` and the rows
@@ -121,7 +121,7 @@ def paged_attention(q: Tensor, k: Tensor, v: Tensor, pages: Tensor, starts: Tens
         ins.append(_node(op, "counts", counts))
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1]) if q.shape and q.shape[-1] else 1.0
-    return Tensor(_active().create(op, ins, scale=_number(op, "scale", scale, above=0.0, high=LARGEST),
+    return Tensor(_active().create(op, ins, scale=_number(op, "scale", scale, low=1 / LARGEST, high=LARGEST),
                                    window=None if window is None else _whole(op, "window", window, 1)))
 
 

@@ -59,3 +59,15 @@ def test_a_reshaped_cache_is_written_once():
 
     program = lower(trace(f, T(10, 4, 72), NEW, PAGES, SEQ))
     assert program.storage(program.graph.outputs[0]) is program.graph.inputs[0]
+
+
+# ---------------------------------------------------------------------------
+# number parameters: fp32 constants of the kernels
+# ---------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("scale", [5e-324, 1e-46, 1e-38, 9e-31, 1.1e30])
+def test_paged_attention_refuses_scales_that_fp32_does_not_hold(scale):
+    """A scale that is 0 in fp32 makes a masked score, -inf, times it NaN."""
+    with pytest.raises(ValueError, match="paged_attention: scale"):
+        trace(lambda q, c, p, s: tj.paged_attention(q, c, c, p, s, scale=scale), T(2, 5, 6, 24), CACHE, PAGES, SEQ)
