@@ -30,10 +30,12 @@ def _node(op: str, name: str, t) -> Node:
     return t.node
 
 
-def _number(op: str, name: str, v, low: float = -math.inf, above: float = -math.inf, high: float = math.inf) -> float:
+def _number(op: str, name: str, v, low: float = -math.inf, above: float = -math.inf, high: float = math.inf,
+            least: float = 0.0) -> float:
+    """``v``, checked: from ``low`` (or past ``above``) to ``high``, and 0 or of at least the size ``least``."""
     if isinstance(v, bool) or not isinstance(v, (int, float)):
         raise TypeError(f"{op}: {name} must be a number, got {type(v).__name__}")
-    if not (math.isfinite(v) and low <= v <= high and v > above):
+    if not (math.isfinite(v) and low <= v <= high and v > above and (v == 0 or abs(v) >= least)):
         raise ValueError(f"{op}: {name} = {v} is out of range")
     return float(v)
 
@@ -59,7 +61,8 @@ def rotary(x: Tensor, positions: Tensor, *, dims: int | None = None, interleaved
     Long contexts: ``factor`` divides every frequency.  With ``original``, the context length the
     model was trained for, it does so by parts: a pair that turns more than ``ramp[1]`` times over
     that length keeps its frequency, one that turns less than ``ramp[0]`` times has it divided, and
-    those between blend linearly.  ``magnitude`` scales the turned values.
+    those between blend linearly.  ``magnitude`` scales the turned values
+    (0, or from 1e-30 to 1e30 in size).
 
     ``inverse`` turns back: with the same arguments it is the gradient, ``dx = rotary(dy, ...,
     inverse=True)``.  Angles are computed in 64 bits, so far positions keep their fraction of a
@@ -78,7 +81,8 @@ def rotary(x: Tensor, positions: Tensor, *, dims: int | None = None, interleaved
     return Tensor(_active().create(
         op, [xn, pn], dims=dims, interleaved=bool(interleaved), base=_number(op, "base", base, low=1 / LARGEST, high=LARGEST),
         factor=_number(op, "factor", factor, low=1 / LARGEST, high=LARGEST), original=None if original is None else _whole(op, "original", original, 1),
-        ramp=ramp, magnitude=_number(op, "magnitude", magnitude, low=-LARGEST, high=LARGEST), inverse=bool(inverse), heads_first=bool(heads_first)))
+        ramp=ramp, magnitude=_number(op, "magnitude", magnitude, low=-LARGEST, high=LARGEST, least=1 / LARGEST),
+        inverse=bool(inverse), heads_first=bool(heads_first)))
 
 
 def paged_write(cache: Tensor, x: Tensor, pages: Tensor, starts: Tensor, counts: Tensor | None = None) -> Tensor:

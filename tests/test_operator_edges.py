@@ -71,3 +71,14 @@ def test_paged_attention_refuses_scales_that_fp32_does_not_hold(scale):
     """A scale that is 0 in fp32 makes a masked score, -inf, times it NaN."""
     with pytest.raises(ValueError, match="paged_attention: scale"):
         trace(lambda q, c, p, s: tj.paged_attention(q, c, c, p, s, scale=scale), T(2, 5, 6, 24), CACHE, PAGES, SEQ)
+
+
+@pytest.mark.parametrize("magnitude", [1e-46, -1e-46, 1e-40, -9e-31])
+def test_rotary_refuses_magnitudes_that_fp32_does_not_hold(magnitude):
+    """1e-46 is 0 in fp32, and 1e-40 keeps half of its digits; 0 itself is one."""
+    def rotary(m):
+        return trace(lambda x, p: tj.rotary(x, p, magnitude=m), NEW, T(2, 5, dt="i32"))
+
+    with pytest.raises(ValueError, match="rotary: magnitude"):
+        rotary(magnitude)
+    assert rotary(0).outputs[0].type == NEW and rotary(-1e-30).outputs[0].type == NEW
