@@ -22,6 +22,7 @@ from ..ir import Node
 from .tracer import Tensor, _active
 
 LARGEST = 1e30          # number parameters become fp32 constants
+SMALLEST_FP32 = 2.0**-149
 
 
 def _node(op: str, name: str, t) -> Node:
@@ -162,5 +163,6 @@ def sample(logits: Tensor, uniform: Tensor, *, temperature=1.0, top_k=None, top_
             low = 0.0 if name in ("temperature", "min_p") else -math.inf
             numbers.append((name, _whole(op, name, v, 1) if name == "top_k" else
                             _number(op, name, v, low=low, above=0.0 if name == "top_p" else -math.inf,
-                                    high=LARGEST if name == "temperature" else 1.0)))
+                                    high=LARGEST if name == "temperature" else 1.0,
+                                    least=SMALLEST_FP32 if name == "temperature" else 0.0)))
     return Tensor(_active().create(op, ins, tensors=tuple(tensors), numbers=tuple(numbers)))

@@ -82,3 +82,15 @@ def test_rotary_refuses_magnitudes_that_fp32_does_not_hold(magnitude):
     with pytest.raises(ValueError, match="rotary: magnitude"):
         rotary(magnitude)
     assert rotary(0).outputs[0].type == NEW and rotary(-1e-30).outputs[0].type == NEW
+
+
+@pytest.mark.parametrize("temperature", [5e-324, 1e-300, 7e-46])
+def test_sample_refuses_temperatures_that_are_zero_in_fp32(temperature):
+    """As 0 they would give the first of several largest logits instead of one of them by its share."""
+    def sample(t):
+        return trace(lambda x, u: tj.sample(x, u, temperature=t), T(3, 50), T(3, dt="f32"))
+
+    with pytest.raises(ValueError, match="sample: temperature"):
+        sample(temperature)
+    for t in (0, 0.0, 1e-38, 1.5e-45):
+        assert sample(t).outputs[0].type == TensorType((3,), DType.i32)
