@@ -210,7 +210,7 @@ template <typename T, unsigned int V, unsigned int SW, bool HELD> struct tj_samp
     top = hi;
     tv = -__builtin_inff();
     ti = 0u;
-    rate = 1.4426950408889634 / (double)fmaxf(temp, 1e-30f);
+    rate = 1.4426950408889634 / (double)temp;      // up to 2^150, in range; not used at 0 and below
     shift = -(double)hi * rate;
     // the buckets cover what has a mass (45 halvings), or the row where that is less
     inv = (float)NB / fmaxf(fminf(45.0f / (float)rate, hi - lo), 1e-30f);
