@@ -684,6 +684,8 @@ class HipProgram:
             ins.append(t)
         if self._written:
             self._check_written(inputs, ins)
+            # autograd refuses what it saved of them before (0.5 us; nothing for inference tensors)
+            torch.autograd.graph.increment_version([ins[i] for i, _ in self._written])
         return ins
 
     def __call__(self, *inputs: torch.Tensor) -> list[torch.Tensor]:

@@ -97,7 +97,9 @@ def paged_write(cache: Tensor, x: Tensor, pages: Tensor, starts: Tensor, counts:
     The write is in place: ``cache`` must be an argument of the traced function (or another
     write's result), contiguous and 16-byte aligned, in no other argument's memory, and the result
     is that very tensor.  Whatever reads the cache in the same function has to read the result, and
-    the result has to be returned or read."""
+    the result has to be returned or read.  Autograd does not record the write; a call moves the
+    tensor's version, as torch's own writes in place do (a captured graph's replays do not), so a
+    backward pass that needs its former values is refused."""
     op = "paged_write"
     ins = [_node(op, "cache", cache), _node(op, "x", x), _node(op, "pages", pages), _node(op, "starts", starts)]
     if counts is not None:

@@ -1,7 +1,9 @@
 """Operators without a GPU: calls at the edge of what they accept."""
 import pytest
+import torch
 
 import tensorjit as tj
+from tensorjit.backends.hip_backend import HipProgram
 from tensorjit.compiler import lower
 from tensorjit.ir import DType, TensorType
 
@@ -94,3 +96,36 @@ def test_sample_refuses_temperatures_that_are_zero_in_fp32(temperature):
         sample(temperature)
     for t in (0, 0.0, 1e-38, 1.5e-45):
         assert sample(t).outputs[0].type == TensorType((3,), DType.i32)
+
+
+# ---------------------------------------------------------------------------
+# calls
+# ---------------------------------------------------------------------------
+
+
+def program_of(fn, *types):
+    """A program's argument checks, on CPU tensors and without its kernels."""
+    program = object.__new__(HipProgram)
+    program.program = lower(trace(fn, *types))
+    program._input_index = {id(n): i for i, n in enumerate(program.program.graph.inputs)}
+    program._out_nodes, program._out_index, program.device_index = [], {}, 0
+    program._init_call_path()
+    program.device_index = -1           # where tensors of the CPU are
+    return program
+
+
+def test_torch_sees_writes_in_place():
+    """What autograd saved of a cache before it was written is refused in the backward pass."""
+    program = program_of(lambda c, x, p, s: tj.paged_write(c, x, p, s), T(10, 4, 3, 24, dt="f32"), T(2, 5, 3, 24, dt="f32"), PAGES, SEQ)
+    cache, new = torch.zeros(10, 4, 3, 24), torch.zeros(2, 5, 3, 24)
+    args = [cache, new, torch.zeros(2, 6, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)]
+    w = torch.ones(24, requires_grad=True)
+    loss = (w * cache).sum()
+    before = [t._version for t in args]
+    program._prepare(args)
+    assert cache._version > before[0] and [t._version for t in args[1:]] == before[1:]
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with torch.inference_mode():
+        args[0] = torch.zeros(10, 4, 3, 24)         # has no counter
+    program._prepare(args)

@@ -69,3 +69,34 @@ def test_sample_small_temperatures(V, size):
     check_sample(x, u, aside=1, temperature=t, top_p=0.8)
     check_sample(x, u, aside=1, temperature=t, top_k=40, min_p=0.01)
     check_sample(x, u, aside=1, temperature=size)
+
+
+# ---------------------------------------------------------------------------
+# writes in place
+# ---------------------------------------------------------------------------
+
+
+def test_torch_sees_writes_in_place():
+    """A call, an eager one and one under capture, moves the version of the cache and of nothing else."""
+    cache, x = normal(6, 4, 2, 8), normal(2, 3, 2, 8, seed=1)
+    pages = torch.arange(6, dtype=torch.int32, device=DEV).reshape(2, 3)
+    starts = torch.tensor([0, 5], dtype=torch.int32, device=DEV)
+    args = (cache, x, pages, starts)
+    f = tj.jit(lambda *a: tj.paged_write(*a))
+    f(*args)
+    w = torch.ones(8, device=DEV, requires_grad=True)
+    loss = (w * cache).sum()
+    before = [t._version for t in args]
+    assert f(*args) is cache
+    assert cache._version > before[0] and [t._version for t in args[1:]] == before[1:]
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    before, graph = cache._version, torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        f(*args)
+    assert cache._version > before
+    with torch.inference_mode():
+        other = cache.clone().zero_()
+        assert f(other, x, pages, starts) is other
+    want = ref.paged_write(torch.zeros(6, 4, 2, 8), x.cpu(), pages.cpu(), starts.cpu())
+    assert torch.equal(other.cpu(), want)
