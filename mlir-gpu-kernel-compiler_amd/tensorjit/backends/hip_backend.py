@@ -142,7 +142,7 @@ def generate_kernel(k: Kernel, idx: int, cfg: MatmulConfig | None = None,
     if k.kind == "colreduce":
         return gen_colreduce(g)
     if k.kind == "operator":
-        return gen_operator(g, alone)
+        return gen_operator(g)
     raise NotImplementedError(k.kind)
 
 

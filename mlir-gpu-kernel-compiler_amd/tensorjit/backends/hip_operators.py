@@ -14,7 +14,6 @@ from ..ir.operators import position_shape
 from ..runtime.autotune import CU_COUNT
 from .common import broadcast_strides, offset_expr
 from .hip_kernels import KernelGen, Launch, _index_type
-from .hip_prelude import CTYPE
 
 THREADS = 256
 # element type of vectors that are converted to and from fp32 whole
@@ -31,7 +30,7 @@ def operand(g: KernelGen, i: int) -> str:
     return g.names[id(g.k.anchor.inputs[i])] + "_p"
 
 
-def gen_operator(g: KernelGen, alone: bool):
+def gen_operator(g: KernelGen):
     op = g.k.anchor.op
     if op == "rotary":
         return gen_rotary(g)
@@ -40,7 +39,7 @@ def gen_operator(g: KernelGen, alone: bool):
     if op == "paged_attention":
         from .hip_paged import gen_paged_attention
 
-        return gen_paged_attention(g, alone)
+        return gen_paged_attention(g)
     if op == "sample":
         from .hip_sample import gen_sample
 

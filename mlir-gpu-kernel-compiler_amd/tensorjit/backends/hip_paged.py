@@ -899,7 +899,7 @@ def _softmax(src: str) -> str:
     return src
 
 
-def gen_paged_attention(g: KernelGen, alone: bool):
+def gen_paged_attention(g: KernelGen):
     n = g.k.anchor
     q, kc = n.inputs[:2]
     dt = q.dtype

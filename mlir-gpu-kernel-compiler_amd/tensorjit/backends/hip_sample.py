@@ -541,7 +541,7 @@ enum { TJ_ALL = 0, TJ_LIST = 1, TJ_CUT = 2 };      // kept: all tokens; top_k of
 template <typename T, unsigned int V, unsigned int N, unsigned int SL, bool HELD> struct tj_sample_split {
   typedef tj_sampler<T, V, N, HELD> Slice;
   typedef tj_sampler<T, V, N * SL, false> Row;
-  static constexpr unsigned int TH = 1024, NB = Slice::NB, SEG = Slice::SEG, LIST = Slice::LIST;
+  static constexpr unsigned int TH = 1024, NB = Slice::NB, SEG = Slice::SEG;
   tj_sample_state* st;
   tj_u64 *ext, *hist, *total, *seg;
   unsigned int* cnt;
@@ -585,7 +585,7 @@ template <typename T, unsigned int V, unsigned int N, unsigned int SL, bool HELD
     s.extremes(hi, lo);
     if (threadIdx.x == 0u) ext[slice] = (tj_u64)__builtin_bit_cast(unsigned int, lo) << 32 | __builtin_bit_cast(unsigned int, hi);
   }
-  __device__ __forceinline__ void b(Slice& s, float u, float temp, int top_k, float top_p, float min_p, int* out) {
+  __device__ __forceinline__ void b(Slice& s, float u, float temp, int top_k, float top_p, float min_p) {
     const unsigned int tid = threadIdx.x;
     const bool count = by_count(temp, top_k), mass = by_mass(temp, top_k, top_p);
     float hi, lo;
@@ -747,7 +747,7 @@ def gen_sample(g: KernelGen):
     row_bytes = 16 + 8 * SL * (1 + 2048 + 1 + THREADS // 64)
     calls = {"a": "p.a(s);"}
     if filtered:
-        calls["b"] = f"p.b(s, {u}, {temp}, {top_k}, {top_p}, {min_p}, out0_p + row);"
+        calls["b"] = f"p.b(s, {u}, {temp}, {top_k}, {top_p}, {min_p});"
     calls["c"] = f"p.c(s, {str(filtered).lower()}, {u}, {temp}, {top_k}, {top_p}, {min_p}, out0_p + row);"
     L, launches = [f"static_assert({split}::BYTES == {row_bytes}u, \"workspace\");"], []
     for i, (which, call) in enumerate(calls.items()):
