@@ -33,26 +33,58 @@ def normal(*shape, dt=torch.float32, seed=0, scale=1.0):
 
 
 def mass_error(logits, temperature):
-    """How far a cumulative mass may be off, of the total, which is at least the largest mass: per token
-    half a step of 2^-43 of that; and of each mass the exponential's 2^-38 and what 64-bit arithmetic
-    makes of the exponent, 2^-52 of the largest logit over the temperature, in either's unit."""
+    """How far one mass may be off, of the largest (half a step of 2^-43) and of itself: the exponential's 2^-38, and what
+    64-bit arithmetic makes of the exponent, 2^-52 of the largest logit over the temperature, in either's unit."""
     x = logits.double()
     x = x[x.isfinite()]
     t = float(torch.as_tensor(temperature, dtype=torch.float64).min())
     size = float(x.abs().max()) / t if x.numel() and t > 0 else 0.0
-    return logits.shape[-1] * 2.0**-44 + 2.0**-38 + size * 2.0**-52
+    return 2.0**-44, 2.0**-38 + size * 2.0**-52
+
+
+def clear_of_borders(logits, uniform, errors, temperature=1.0, top_k=None, top_p=None, min_p=None):
+    """Whether each row's choice is the same wherever its masses lie within their errors.  A sum of V masses is off
+    by V times the first error and once the second, of the row's total, which is at least the largest mass; two
+    sums are compared.  ``min_p`` is compared with one mass."""
+    step, relative = errors
+    two_sums = 2 * (logits.shape[-1] * step + relative)
+
+    def at(p, r):
+        return None if p is None else float(p[r]) if isinstance(p, torch.Tensor) else float(p)
+
+    clear = []
+    for r, x in enumerate(logits.detach().cpu().double()):
+        t, k, tp, mp = (at(v, r) for v in (temperature, top_k, top_p, min_p))
+        if not t > 0:
+            clear.append(True)
+            continue
+        p = torch.exp((x - x.max()) / t)
+        order = torch.argsort(x, descending=True, stable=True)
+        keep, ok = order[:int(k)] if k is not None and k > 0 else order, True
+        if tp is not None and tp < 1:
+            upto = p[keep].cumsum(0)
+            ok &= bool(((upto[:-1] - tp * upto[-1]).abs() > two_sums * upto[-1]).all())
+            keep = keep[:1 + int((upto < tp * upto[-1]).sum())]
+        if mp is not None:
+            others = p[keep][p[keep] < 1]
+            ok &= bool(((others - mp).abs() > step + relative * others).all())
+            keep = keep[p[keep] >= mp]
+        upto = p[keep.sort().values].cumsum(0)
+        ok &= bool(((upto[:-1] - float(uniform[r]) * upto[-1]).abs() > two_sums * upto[-1]).all())
+        clear.append(ok)
+    return torch.tensor(clear)
 
 
 def check_sample(logits, uniform, aside=0, **params):
-    """``aside``: rows that may stand nearer to a border than two sums (of either side) may be off."""
+    """``aside``: rows that may stand on a border."""
     tensors = {n: p for n, p in params.items() if isinstance(p, torch.Tensor)}
 
     def fn(x, u, *rest):
         return tj.sample(x, u, **{**params, **dict(zip(tensors, rest))})
 
     got = tj.jit(fn)(logits, uniform, *tensors.values())
-    want, margin = ref.sample(logits, uniform, **params)
-    clear = margin > 2 * mass_error(logits, params.get("temperature", 1.0))
+    want = ref.sample(logits, uniform, **params)[0]
+    clear = clear_of_borders(logits, uniform, mass_error(logits, params.get("temperature", 1.0)), **params)
     assert int((~clear).sum()) <= aside
     assert torch.equal(got.cpu()[clear], want[clear])
     return got
@@ -69,6 +101,57 @@ def test_sample_small_temperatures(V, size):
     check_sample(x, u, aside=1, temperature=t, top_p=0.8)
     check_sample(x, u, aside=1, temperature=t, top_k=40, min_p=0.01)
     check_sample(x, u, aside=1, temperature=size)
+
+
+def two_values(dt, R, V, top_k=None, top_p_at=None, min_p=None):
+    """Rows with every seventh logit 1 and the others 0, uniforms in the middle of a kept token's
+    share, and ``top_p`` in the middle of the share of the token ``top_p_at`` (in order): no row
+    stands on a border.  The filters in float64, from counts alone."""
+    x = torch.zeros(R, V)
+    x[:, ::7] = 1.0
+    p = torch.exp(x[0].double() - 1.0)
+    order = torch.cat([torch.arange(0, V, 7), torch.tensor([i for i in range(V) if i % 7])])
+    kept, top_p = order[:top_k], None
+    if top_p_at is not None:
+        cum = p[kept].cumsum(0)
+        top_p = float(((cum[top_p_at] - p[kept[top_p_at]] / 2) / cum[-1]).float())
+        kept = kept[:top_p_at + 1]
+    if min_p is not None:
+        kept = kept[p[kept] >= min_p]
+    kept = kept.sort().values
+    cum = p[kept].cumsum(0)
+    at = torch.tensor([0, len(kept) - 1, len(kept) // 2, len(kept) // 3])[:R]
+    u = ((cum[at] - p[kept[at]] / 2) / cum[-1]).float()
+    # as one value per row, those that mean all tokens among them: one program serves every case
+    params = dict(top_k=torch.full((R,), top_k or 0, dtype=torch.int32, device=DEV),
+                  top_p=torch.full((R,), top_p or 1.0, device=DEV), min_p=torch.full((R,), min_p or 0.0, device=DEV))
+    return x.to(DEV, dt), u.to(DEV), params, kept[at]
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("V", [9001, 100003, 151001])
+def test_sample_borders_within_equal_logits(dt, V):
+    """A filter ends among thousands of equal logits, more than are ranked: by their keys' digits and
+    then by index, for rows of one workgroup and rows split over several.  Every row is compared."""
+    ones = -(-V // 7)
+    for kwargs in (dict(top_k=300), dict(top_k=ones), dict(top_k=V // 3), dict(top_k=V - 1), dict(top_p_at=200), dict(top_p_at=ones - 1),
+                   dict(top_p_at=ones + 4321), dict(top_k=V // 2, top_p_at=V // 3), dict(top_k=V // 2, top_p_at=77),
+                   dict(top_k=V // 3, min_p=0.5), dict(top_p_at=V // 2, min_p=0.3), dict(min_p=0.5)):
+        x, u, params, want = two_values(dt, 4, V, **kwargs)
+        got = check_sample(x, u, **params)
+        assert got.tolist() == want.tolist(), kwargs
+
+
+@pytest.mark.parametrize("V", [100003, 1 << 20])
+def test_sample_long_rows_by_the_bound_of_their_length(V):
+    """Cumulative masses are off by up to V half steps, so which rows are set aside follows from V.  At 2^20
+    tokens a nucleus of 0.999 ends among masses smaller than that; one row of three is always compared."""
+    R = 3
+    x, u = normal(R, V, scale=3.0), torch.rand(R, device=DEV, generator=gen(1))
+    k = torch.tensor([0, 700, V // 4], dtype=torch.int32, device=DEV)
+    p = torch.tensor([0.95, 0.5, 0.999], device=DEV)
+    for params in (dict(), dict(top_k=k), dict(top_p=p), dict(top_k=k, top_p=p), dict(min_p=1e-4)):
+        check_sample(x, u, aside=2, **params)
 
 
 # ---------------------------------------------------------------------------
