@@ -318,6 +318,7 @@ FEW16 = r"""
   int lo[QT], hi[QT];
   bool sees[QT];
   float m_run[QT], l_run[QT];
+  bool far = false;                  // see SOFTMAX
   tj_f32x4 o[QT][NU];
 #pragma unroll
   for (int x = 0; x < QT; ++x) {
@@ -390,8 +391,8 @@ FEW16 = r"""
       tj_u32x4 pw;
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
-        const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[w / 2][w % 2 * 2], CS, -m_run[x]));
-        const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[w / 2][w % 2 * 2 + 1], CS, -m_run[x]));
+        const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[w / 2][w % 2 * 2], CS, -ref));
+        const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[w / 2][w % 2 * 2 + 1], CS, -ref));
         pw[w] = PACK2(e0, e1);
         l_run[x] = PAIR_SUM(pw[w], l_run[x]);
       }
@@ -467,18 +468,30 @@ STORE_FEW = r"""
 
 # Lazy rescale: the reference moves only where a score passes it by 2^8.  The sums are those of the
 # probabilities as they were rounded for the product with V, so that the weights sum to one.
+# An exponent is fma(s, CS, -ref), where the reference is a rounded product: together off by half a last place
+# of the reference, the same for all keys of a row.  From 2^27 on that would be a power that no type holds, so
+# far references take rounded products on both sides.
 SOFTMAX = r"""
+      float ref;
       {
+#pragma clang fp contract(off)
         float mx = s[0][0];
 #pragma unroll
         for (int e = 1; e < 4 * (TILES); ++e) mx = fmaxf(mx, s[e / 4][e % 4]);
         const float mb = mx * CS;
-        if (__builtin_amdgcn_ballot_w64(mb > m_run[X] + 8.0f)) {
+        if (__builtin_amdgcn_ballot_w64(mb - m_run[X] > 8.0f)) {
           const float mn = fmaxf(m_run[X], tj_quad_max(mb)), f = __builtin_amdgcn_exp2f(m_run[X] - mn);
           l_run[X] *= f;
 #pragma unroll
           for (unsigned int u = 0; u < (UNITS); ++u) o[X][u] *= f;
           m_run[X] = mn;
+          far |= __builtin_amdgcn_ballot_w64(__builtin_fabsf(mn) > 0x1p20f && mn != LOWEST) != 0ul;
+        }
+        ref = m_run[X];
+        if (far) {
+#pragma unroll
+          for (int e = 0; e < 4 * (TILES); ++e) s[e / 4][e % 4] = (s[e / 4][e % 4] * CS - ref) * (1.0f / CS);
+          ref = 0.0f;
         }
       }
 """
@@ -546,6 +559,7 @@ CHUNK16 = r"""
   int lo[QT], hi[QT];
   bool sees[QT];
   float m_run[QT], l_run[QT];
+  bool far = false;                  // see SOFTMAX
   tj_f32x4 o[QT][NU];
   const unsigned int rw = r0 + wave * (16u * QT);
 #pragma unroll
@@ -618,8 +632,8 @@ QK_SCHED
           tj_u32x4 pw;
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
-            const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2u * h + w / 2][w % 2 * 2], CS, -m_run[x]));
-            const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2u * h + w / 2][w % 2 * 2 + 1], CS, -m_run[x]));
+            const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2u * h + w / 2][w % 2 * 2], CS, -ref));
+            const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2u * h + w / 2][w % 2 * 2 + 1], CS, -ref));
             pw[w] = PACK2(e0, e1);
             l_run[x] = PAIR_SUM(pw[w], l_run[x]);
           }
@@ -734,6 +748,7 @@ DIRECT32 = r"""
   int lo[QT], hi[QT];
   bool sees[QT];
   float m_run[QT], l_run[QT];
+  bool far = false;                  // see SOFTMAX
   tj_f32x4 o[QT][NU];
   const unsigned int rw = r0 + (KW == 1 ? wave * (16u * QT) : 0u);
 #pragma unroll
@@ -804,7 +819,7 @@ DIRECT32 = r"""
       SOFTMAX(x, 1, NU)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        s[0][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][e], CS, -m_run[x]));
+        s[0][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][e], CS, -ref));
         l_run[x] += s[0][e];
       }
     }

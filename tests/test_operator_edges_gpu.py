@@ -183,3 +183,50 @@ def test_torch_sees_writes_in_place():
         assert f(other, x, pages, starts) is other
     want = ref.paged_write(torch.zeros(6, 4, 2, 8), x.cpu(), pages.cpu(), starts.cpu())
     assert torch.equal(other.cpu(), want)
+
+
+# ---------------------------------------------------------------------------
+# attention
+# ---------------------------------------------------------------------------
+
+
+def caches(B, L, page, KV, D, dt, seed=0, scale=1.0):
+    """K, V and a page table whose sequences own distinct, shuffled pages."""
+    P = -(-L // page)
+    pages = torch.randperm(B * P, device=DEV, generator=gen(seed)).reshape(B, P).to(torch.int32)
+    return normal(B * P, page, KV, D, dt=dt, seed=seed, scale=scale), normal(B * P, page, KV, D, dt=dt, seed=seed + 1), pages
+
+
+@pytest.mark.parametrize("dt, size", [(torch.float16, 3e3), (torch.float16, 1e4), (torch.bfloat16, 3e3), (torch.bfloat16, 1e5),
+                                      (torch.bfloat16, 1e15), (torch.float32, 1e5), (torch.float32, 1e15)])
+@pytest.mark.parametrize("S", [1, 6, 70])
+@pytest.mark.parametrize("negative", [False, True])
+def test_scores_of_any_size(dt, size, S, negative):
+    """Scores that fp32 holds give what they give in 64 bits: the value of the largest one's key, where the next is
+    20 and more below it, whatever 64 products in fp32 may be off."""
+    B, L, D = 2, 300, 64
+    k, v, pages = caches(B, L, 16, 2, D, dt, scale=size)
+    if negative:                     # every score far below zero
+        k[..., 0] = 4.0 * size
+    q = normal(B, S, 6, D, dt=dt, seed=5, scale=size)
+    if negative:
+        q[..., 0] = -6.0 * size
+    assert q.isfinite().all() and k.isfinite().all()
+    starts = torch.tensor([L - S, 40], dtype=torch.int32, device=DEV)
+    got = tj.jit(lambda *a: tj.paged_attention(*a))(q, k, v, pages, starts)
+    compared = 0
+    for b in range(B):
+        ks, vs = (t[pages[b].long()].flatten(0, 1).double() for t in (k, v))
+        for i in range(S):
+            n = int(starts[b]) + i + 1
+            for h in range(6):
+                x = q[b, i, h].double()
+                s, terms = ks[:n, h // 3] @ x / 8, ks[:n, h // 3].abs() @ x.abs() / 8
+                top = s.topk(2)
+                if float(top.values[0] - top.values[1]) < 20 + 2 * 66 * 2.0**-24 * float(terms.max()):
+                    continue
+                compared += 1
+                want = vs[top.indices[0], h // 3]
+                assert bool(((got[b, i, h].double() - want).abs() <= torch.finfo(dt).eps * want.abs() + 2.0**-24).all()), (b, i, h)
+    assert compared > B * S * 3
+    assert got.isfinite().all()
