@@ -31,6 +31,7 @@ from .hip_operators import operand, operator_name
 from .hip_prelude import CTYPE
 
 LOG2E = 1.4426950408889634
+FP16_SHIFT = 7.0        # see SOFTMAX
 FEW_ROWS = 32
 FEW_TILES = 3 * CU_COUNT // 2    # see few_rows()
 WIDE_TILES = CU_COUNT            # see wide_tiles()
@@ -466,8 +467,10 @@ STORE_FEW = r"""
         }
 """
 
-# Lazy rescale: the reference moves only where a score passes it by 2^8.  The sums are those of the
-# probabilities as they were rounded for the product with V, so that the weights sum to one.
+# Lazy rescale: the reference moves only where a score passes it by 2^8.  The 16-bit types round the
+# probabilities to theirs, as the product with V on MFMAs takes them (half a step each); the sums are those of
+# the rounded ones, so that the weights sum to one.  fp16 ones stand 2^SHIFT higher, up to 2^15: fp16 has steps
+# of 2^-24 below 2^-14, and without SHIFT a weight under 2^-25 of the largest came to nothing, however many.
 # An exponent is fma(s, CS, -ref), where the reference is a rounded product: together off by half a last place
 # of the reference, the same for all keys of a row.  From 2^27 on that would be a power that no type holds, so
 # far references take rounded products on both sides.
@@ -479,8 +482,8 @@ SOFTMAX = r"""
 #pragma unroll
         for (int e = 1; e < 4 * (TILES); ++e) mx = fmaxf(mx, s[e / 4][e % 4]);
         const float mb = mx * CS;
-        if (__builtin_amdgcn_ballot_w64(mb - m_run[X] > 8.0f)) {
-          const float mn = fmaxf(m_run[X], tj_quad_max(mb)), f = __builtin_amdgcn_exp2f(m_run[X] - mn);
+        if (__builtin_amdgcn_ballot_w64(mb - m_run[X] > 8.0f + SHIFT)) {
+          const float mn = fmaxf(m_run[X], tj_quad_max(mb) - SHIFT), f = __builtin_amdgcn_exp2f(m_run[X] - mn);
           l_run[X] *= f;
 #pragma unroll
           for (unsigned int u = 0; u < (UNITS); ++u) o[X][u] *= f;
@@ -969,7 +972,7 @@ def gen_paged_attention(g: KernelGen):
             *([f"  typedef {_index_type(2 * places)} pos_t;          // places in the list of all blocks"] if few else [])]
     if not f32:
         text.append(f"  constexpr unsigned int KP = {KP}u, VP = {VP}u; constexpr bool BF = {str(bf).lower()};")
-    text += [f"  constexpr float CS = {cs!r}f, LOWEST = -3.402823466e+38f;",
+    text += [f"  constexpr float CS = {cs!r}f, LOWEST = -3.402823466e+38f, SHIFT = {FP16_SHIFT if dt == DType.f16 else 0.0}f;",
              *(f"  const {T}* __restrict__ {nm} = {operand(g, i)};" for i, nm in enumerate(("q_p", "k_p", "v_p"))),
              f"  const int* __restrict__ pages_p = {operand(g, 3)};", f"  const int* __restrict__ starts_p = {operand(g, 4)};",
              "  const unsigned int tid = threadIdx.x, lane = tid % 64u, wave = __builtin_amdgcn_readfirstlane(tid / 64u);",

@@ -230,3 +230,29 @@ def test_scores_of_any_size(dt, size, S, negative):
                 assert bool(((got[b, i, h].double() - want).abs() <= torch.finfo(dt).eps * want.abs() + 2.0**-24).all()), (b, i, h)
     assert compared > B * S * 3
     assert got.isfinite().all()
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("S, G, L", [(1, 4, 40000), (24, 4, 5000), (3, 2, 5000)])
+@pytest.mark.parametrize("lead", [5.0, 12.0, 18.0])
+def test_many_keys_behind_one_that_leads(dt, S, G, L, lead):
+    """One key's score is above all others by ``lead`` and its value is zero, so the output is what the small
+    weights of the others add up to.  fp16 holds a weight (at most half a step of its own size, as in every
+    bound) or half of 2^-31 of the largest, which the reference of a row is never above."""
+    D, page, KV = 64, 16, 2
+    P = -(-L // page)
+    k, v = torch.zeros(P, page, KV, D, device=DEV), 1.0 + torch.rand(P, page, KV, D, device=DEV, generator=gen(1))
+    k[..., 1] = torch.randn(P, page, KV, device=DEV, generator=gen(2)) * 0.25      # other scores: -0.25 .. 0.25 or so
+    k[L // 3 // page, L // 3 % page, :, 0] = 8.0
+    v[L // 3 // page, L // 3 % page] = 0.0
+    q = torch.zeros(2, S, KV * G, D, device=DEV)
+    q[..., 0], q[..., 1] = lead, 1.0
+    q, k, v = (t.to(dt) for t in (q, k, v))
+    pages = torch.arange(P, dtype=torch.int32, device=DEV).expand(2, P).contiguous()
+    starts = torch.tensor([L - S, L // 2], dtype=torch.int32, device=DEV)
+    got = tj.jit(lambda *a: tj.paged_attention(*a))(q, k, v, pages, starts).cpu().double()
+    want, bound = ref.paged_attention(q, k, v, pages, starts)
+    if dt == torch.float16:
+        n = starts.cpu().double()[:, None, None, None] + S
+        bound = bound + n * 2.0**-32 * float(v.abs().max()) + 2.0**-25      # and the output's own smallest step
+    assert bool((want > 0).all()) and bool(((got - want).abs() <= bound).all()), float(((got - want).abs() / want).max())
