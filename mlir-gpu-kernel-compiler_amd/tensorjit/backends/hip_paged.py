@@ -14,8 +14,8 @@ Two work divisions of a 256-lane workgroup:
   8.5 us, which is latency.
 * a chunk: the four waves take 16 or 32 rows each and share every key block through LDS (fp32:
   through the L1, whose rate is enough at fp32's MFMA rate).  Bound by the MFMAs and the softmax,
-  which two waves of a SIMD overlap: 4 x 1024 tokens behind 8000 0.85 to 0.93 PFLOP/s, behind ragged 1500
-  to 3000 220 us, 0.72; fp32 91 TFLOP/s.
+  which two waves of a SIMD overlap: 4 x 1024 tokens behind 8000 0.92 PFLOP/s (pages of 16) and 0.95 (of 64),
+  behind ragged 1500 to 3000 209 to 245 us by the box, 0.70 to 0.82; fp32 87 TFLOP/s.
 
 Either is also split over the keys where there are too few workgroups; the last workgroup of a
 tile to finish joins the parts.  Lengths are data, so a launch has as many parts as its page table
@@ -37,7 +37,9 @@ FEW_TILES = 3 * CU_COUNT // 2    # see few_rows()
 WIDE_TILES = CU_COUNT            # see wide_tiles()
 FEW_BLOCK = 32          # keys that a wave takes at a time
 LEAST_CHUNK_KEYS = 256  # see chunk_parts()
-CHUNK_GROUPS = FEW_GROUPS = 2 * CU_COUNT        # as many as are resident
+# As many as are resident; of few rows with heads over 128 half of them, by their LDS and registers, so those
+# run in two rounds (48 tokens over 4000 to 8000, 8 heads of 256, bf16: 393 us, 6.2 TB/s).
+CHUNK_GROUPS = FEW_GROUPS = 2 * CU_COUNT
 # Few rows: blocks that a workgroup takes at least, and the blocks' worth of time that a tile takes
 # before its first.  us at 8, 8 / 4, 0, 32:8 heads of 128: 8 x 4000 keys 21.6 / 24.4, 1 x 8000 12.8 / 17-19.
 FEW_LEAST = FEW_OVERHEAD = 8

@@ -6,7 +6,9 @@ its last member: a value and the index behind the last kept token of that value.
 mass) reaches a target, without sorting: a histogram of the weights over the distance from the
 row's largest logit names the bucket, and the tokens of that bucket alone are ranked against each
 other.  ``locate`` then walks the kept masses in index order.  Masses are integers (``2 ** 43`` for
-the largest logit), so sums do not depend on their order and no two runs differ.
+the largest logit), so sums do not depend on their order and no two runs differ.  A sum of V masses is off by
+V half steps, 2^-44 of the largest each (together 2^-28 of it for 2^16 tokens, 2^-24 for 2^20), and by the
+exponential's 2^-38 of itself.
 """
 from __future__ import annotations
 
@@ -151,7 +153,7 @@ template <typename T, unsigned int V, unsigned int SW, bool HELD> struct tj_samp
   // fp64, which costs as much per operation as fp32 here: a mass off by 2^-24 would move a border
   // between two tokens often enough to see (10^4 tokens: one row in 10^4).  2^y = 2^n 2^f, the latter 1 + f
   // times the polynomial that interpolates (2^f - 1) / f at the 8 Chebyshev points of |f| <= 1/2
-  // (relative error under 2^-38).
+  // (relative error under 2^-38; y itself is off by 2^-53 of top / temperature, as in any 64-bit form).
   __device__ __forceinline__ tj_u64 mass(float v) const {
     const double y = __builtin_fmax(__builtin_fma((double)v, rate, shift), -100.0);
     const double n = __builtin_rint(y), f = y - n;
@@ -702,9 +704,13 @@ def sweeps_of(V: int, vec: int) -> int:
 def slices(rows: int, sweeps: int, top_k: bool) -> tuple[int, int]:
     """(slices of a row, sweeps of a slice); one slice: the row is a single workgroup's, in one launch.
 
-    Splitting takes two launches more, each joined by a row's last workgroup.  us, split / one workgroup
+    Splitting takes up to two launches more; those of histograms and of masses are joined by a row's last
+    workgroup.  us, split / one workgroup
     per row: without top-k (masses of every logit) bf16 1 x 32000 19 / 23, 1 x 128000 30 / 73, 64 x 32000
-    26 / 34, 64 x 128000 52 / 113, 384 x 128000 162 / 205, 2048 x 128000 721 / 826, but fp32 256 x 20000 48 / 31; with top-k (counts, then
+    26 / 34, 64 x 128000 52 / 113, 384 x 128000 162 / 205, 2048 x 128000 721 / 826, fp32 128 x 50257 44 / 55, 300 x 100000
+    148 / 178, but 256 x 20000 48 / 31.  Past 128 rows fp32 gains nothing where the rows alone fill the CUs evenly: 512 x 100000
+    206 / 204, 1024 x 100000 388 / 385, and 50257 loses, 256 rows 69 / 61, 512 120 / 114, 1024 214 / 207, 4096 862 / 777;
+    300 x 100000 in three slices took 140.  With top-k (counts, then
     few masses) bf16 1 x 128000 22 / 37, fp32 16 x 50257 22 / 23, 64 x 100003 32 / 47, 128 x 100003 48 / 51, but 64 x 32000
     24 / 18.  A workgroup for each CU: 256, 512, 768 of them 32, 38, 39 (64 x 100003, top-k); a slice
     of 1, 2, 4 sweeps 25, 22, 23 (16 x 50257, top-k) and 30, 32, 37 (1 x 128000, no top-k)."""

@@ -121,7 +121,12 @@ def paged_attention(q: Tensor, k: Tensor, v: Tensor, pages: Tensor, starts: Tens
     that sees no key gives zeros, and so do one whose scores are all ``-inf`` and the rows
     ``i >= counts[b]``.  Rows of the caches that no
     query of a sequence sees are not read, and an infinity or a NaN in ``v`` reaches the queries that
-    see its position, and no others."""
+    see its position, and no others.
+
+    Scores and sums are fp32.  With 16-bit caches each weight is rounded to their type before it meets
+    ``v``, as in dense attention, and the result once more: an error of 1.3 to 1.4 times that of fp32
+    weights (relative to the output 2.3e-3 for 1.7e-3 in bf16, 2.9e-4 for 2.1e-4 in fp16, random data).
+    fp16 holds no weight under 2^-32 of a row's largest."""
     op = "paged_attention"
     ins = [_node(op, n, t) for n, t in (("q", q), ("k", k), ("v", v), ("pages", pages), ("starts", starts))]
     if counts is not None:
@@ -151,7 +156,9 @@ def sample(logits: Tensor, uniform: Tensor, *, temperature=1.0, top_k=None, top_
     row.  A row with nothing but those gives -1.
 
     Masses are summed as integers (steps of ``2 ** -43`` of the largest), so the choice does not
-    depend on any order of summation."""
+    depend on any order of summation.  Of V tokens it is that of 64-bit arithmetic unless a threshold
+    stands nearer to one of their cumulative masses than V ``2 ** -44`` of the largest mass and
+    ``2 ** -38`` of the sum."""
     op = "sample"
     ins = [_node(op, "logits", logits), _node(op, "uniform", uniform)]
     tensors, numbers = [], []
