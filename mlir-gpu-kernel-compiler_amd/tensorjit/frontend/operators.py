@@ -17,6 +17,7 @@ program is compiled for ``S``, and lengths are data.
 from __future__ import annotations
 
 import math
+import struct
 
 from ..ir import Node
 from .tracer import Tensor, _active
@@ -31,12 +32,17 @@ def _node(op: str, name: str, t) -> Node:
     return t.node
 
 
+def _zero(v) -> bool:
+    """By its bits: where a library has the process flush denormals, they compare equal to 0."""
+    return struct.pack("<d", abs(v)) == bytes(8)
+
+
 def _number(op: str, name: str, v, low: float = -math.inf, above: float = -math.inf, high: float = math.inf,
             least: float = 0.0) -> float:
     """``v``, checked: from ``low`` (or past ``above``) to ``high``, and 0 or of at least the size ``least``."""
     if isinstance(v, bool) or not isinstance(v, (int, float)):
         raise TypeError(f"{op}: {name} must be a number, got {type(v).__name__}")
-    if not (math.isfinite(v) and low <= v <= high and v > above and (v == 0 or abs(v) >= least)):
+    if not (math.isfinite(v) and low <= v <= high and v > above and (abs(v) >= least or _zero(v))):
         raise ValueError(f"{op}: {name} = {v} is out of range")
     return float(v)
 

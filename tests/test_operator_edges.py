@@ -94,8 +94,22 @@ def test_sample_refuses_temperatures_that_are_zero_in_fp32(temperature):
 
     with pytest.raises(ValueError, match="sample: temperature"):
         sample(temperature)
-    for t in (0, 0.0, 1e-38, 1.5e-45):
+    for t in (0, 0.0, -0.0, 1e-38, 1.5e-45):
         assert sample(t).outputs[0].type == TensorType((3,), DType.i32)
+
+
+def test_refusals_do_not_depend_on_how_denormals_are_handled():
+    """A library built with -ffast-math has its process flush them (this repository's oracle is one)."""
+    tiny = 5e-324
+    flushed = tiny * 1.0 == 0.0
+    torch.set_flush_denormal(True)
+    try:
+        with pytest.raises(ValueError, match="sample: temperature"):
+            trace(lambda x, u: tj.sample(x, u, temperature=tiny), T(3, 50), T(3, dt="f32"))
+        with pytest.raises(ValueError, match="rotary: magnitude"):
+            trace(lambda x, p: tj.rotary(x, p, magnitude=-tiny), NEW, T(2, 5, dt="i32"))
+    finally:
+        torch.set_flush_denormal(flushed)
 
 
 # ---------------------------------------------------------------------------
